@@ -227,8 +227,9 @@ def token_log_probs_forward(logits: torch.Tensor, tokens: torch.Tensor, temperat
     lead = logits.shape[:-1]
     tokens = _tokens(tokens, "tokens", lead, logits)
     device = logits.device
-    out = torch.empty((2, *lead), dtype=torch.float32, device=device)
-    log_probs, entropy = out[0], out[1]
+    # apart: views of one tensor could not be changed in place once autograd returns them
+    log_probs = torch.empty(lead, dtype=torch.float32, device=device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=device)
     stats = torch.empty((*lead, 2), dtype=torch.float32, device=device)
     top = int(top)
     values = index = None
