@@ -9,13 +9,14 @@
 // are cut into slices, whose (m, s, t) a second kernel joins: joining to a larger maximum, x higher in
 // the units of d, turns s into s 2^-x and t into 2^-x (t - x s).
 //
-// The most likely tokens. The count-th largest of the threads' largest logits (cut to their upper 16
-// bits, bisected by one wave; for few alternatives, of the waves' one to three largest) is a bound that
-// at least `count` logits reach. The vectors whose largest logit reaches it, few more than count of
-// them, are listed in LDS and read again, the logits that reach it listed too, and each one's rank is
-// the number of those before it (larger, or equal and of a lower index). Where more reach it than LDS
-// holds (many equal logits, or large ones crowded into few threads), the exact count-th one is found
-// first, by bisection of its value and then of its index.
+// The most likely tokens. About the count-th largest of the threads' largest logits (bisected by one
+// wave; for few alternatives, of the waves' one to three largest) is a bound that at least `count`
+// logits reach. The vectors whose largest logit reaches it, few more than count of them, are listed in
+// LDS and read again, the logits that reach it listed too, and each one's rank is the number of those
+// before it (larger, or equal and of a lower index). Bound and largest logits are compared in full, so
+// an offset that a row's logits have in common changes nothing. Where more reach the bound than LDS
+// holds (many equal logits, fewer finite ones than alternatives, or large ones crowded into few
+// threads), the exact count-th one is found first, by bisection of its value and then of its index.
 //
 // What bounds it: reading the logits (6.4 TB/s for 8192 rows of 32000 bf16 without alternatives) and,
 // with the gradient, writing as much (5.6 TB/s); a large copy runs at 6.15. With alternatives
@@ -275,22 +276,56 @@ struct RowRegisters {
     }
 };
 
-// The largest logit of each of a thread's vectors, its upper 16 bits: all of a 16-bit logit. Cutting
-// the lower half off keeps the order, so a vector whose cut maximum is below the cut bound holds
-// nothing that reaches the bound.
-template <int NV>
+// The largest logit of each of a thread's vectors of a 16-bit type, as it is: two to a register.
+template <typename T, int NV>
 struct VectorTops {
+    uint32_t two[(NV + 1) / 2];
+    __device__ __forceinline__ void set(int i, float v) {
+        const uint32_t b = __builtin_bit_cast(uint16_t, (store_t<T>)v);
+        two[i / 2] = i % 2 ? (two[i / 2] & 0xffffu) | b << 16 : b;
+    }
+    __device__ __forceinline__ float get(int i, const u32x4 &) const {
+        return (float)__builtin_bit_cast(store_t<T>, (uint16_t)(i % 2 ? two[i / 2] >> 16 : two[i / 2]));
+    }
+};
+
+template <int NV>
+struct VectorTops<BF16, NV> {
     uint32_t two[(NV + 1) / 2];
     __device__ __forceinline__ void set(int i, float v) {
         const uint32_t b = __float_as_uint(v);
         two[i / 2] = i % 2 ? (two[i / 2] & 0xffffu) | (b & 0xffff0000u) : b >> 16;
     }
-    __device__ __forceinline__ float get(int i) const {
+    __device__ __forceinline__ float get(int i, const u32x4 &) const {
         return __uint_as_float(i % 2 ? two[i / 2] & 0xffff0000u : two[i / 2] << 16);
     }
 };
 
-static __device__ __forceinline__ float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+// f32: one to a register. From thirteen vectors on that would spill (4096 x 25000 with 8 alternatives: 71
+// us, and 67 this way), and the four logits are compared again.
+template <int NV>
+struct VectorTops<F32, NV> {
+    static constexpr bool kKept = NV <= 8;
+    float one[kKept ? NV : 1];
+    __device__ __forceinline__ void set(int i, float v) {
+        if (kKept) one[i] = v;
+    }
+    __device__ __forceinline__ float get(int i, const u32x4 &x) const { return kKept ? one[i] : vector_max(x, F32()); }
+};
+
+// A logit's place in the order of its type, 32 or 16 bits, at least 1, and back.
+static __device__ __forceinline__ uint32_t key_of(float v, F32) { return order_of(v); }
+static __device__ __forceinline__ uint32_t key_of(float v, BF16) { return order_of(v) >> 16; }
+static __device__ __forceinline__ uint32_t key_of(float v, F16) {
+    const uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)(v + 0.0f));
+    return b & 0x8000u ? b ^ 0xffffu : b | 0x8000u;
+}
+
+static __device__ __forceinline__ float of_key(uint32_t k, F32) { return of_order(k); }
+static __device__ __forceinline__ float of_key(uint32_t k, BF16) { return of_order(k << 16); }
+static __device__ __forceinline__ float of_key(uint32_t k, F16) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(k & 0x8000u ? k ^ 0x8000u : k ^ 0xffffu));
+}
 
 // A place in a list in LDS for every lane with `in`, or -1; the list's length is *length.
 static __device__ __forceinline__ int append(bool in, int *length) {
@@ -369,11 +404,11 @@ static __device__ __forceinline__ void find_bound(const store_t<T> *z, int len, 
 // logits and the largest of all of them, most: the row's. The lists' order depends on the waves'
 // timing, the ranks do not.
 template <typename T, int THREADS, int NV, typename Put>
-static __device__ __forceinline__ void find_top(const VectorTops<NV> &tops, const store_t<T> *z, int len, int skew, int count,
-                                                float best, float most, RowLds<THREADS, true> &lds, Put put) {
+static __device__ __forceinline__ void find_top(RowRegisters<T, THREADS, NV> &r, const VectorTops<T, NV> &tops, const store_t<T> *z,
+                                                int len, int count, float best, float most, RowLds<THREADS, true> &lds, Put put) {
     using Lds = RowLds<THREADS, true>;
     constexpr int V = Type<T>::kVec, kWaves = THREADS / kWave;
-    const int tid = row_thread<THREADS>(), lane = tid % kWave, wave = tid / kWave;
+    const int skew = r.skew, tid = row_thread<THREADS>(), lane = tid % kWave, wave = tid / kWave;
     float bound = -INFINITY;
     if (tid == 0) lds.vectors = lds.logits = 0;
     const int j = (count + kWaves - 1) / kWaves, n = j * kWaves;
@@ -400,54 +435,86 @@ static __device__ __forceinline__ void find_top(const VectorTops<NV> &tops, cons
         // A short row gives too few threads' bests for a bound: there every logit stands for itself, for
         // twice the time (65536 rows of 1000 bf16 with 64 alternatives take 244 us, 432 this way; with
         // 128 they take 495 us this way, 1143 with the exact search that a bound of -inf leads to).
-        constexpr int kShort = kWaves == 4 && NV <= 8 ? 4 * Lds::kLogits : 0;  // 16-bit keys where the list will be
+        constexpr bool kWide = sizeof(store_t<T>) == 4;  // a key fills a word, or half of one
+        constexpr int kWords = Lds::kLogits * 2;         // of the keys where the list will be
+        constexpr int kShort = kWaves == 4 && NV <= 8 ? kWords * (kWide ? 1 : 2) : 0;
         const bool each = kShort > 0 && len <= kShort && 2 * len < 3 * V * count;
-        uint16_t *keys = reinterpret_cast<uint16_t *>(lds.key);
         if (each) {
-            for (int e = tid; e < kShort; e += THREADS) keys[e] = e < len ? (uint16_t)(order_of(Type<T>::load(z + e)) >> 16) : 0;
+            for (int e = tid; e < kShort; e += THREADS) {
+                const uint32_t key = e < len ? key_of(Type<T>::load(z + e), T()) : 0;
+                if (kWide) reinterpret_cast<uint32_t *>(lds.key)[e] = key;
+                else reinterpret_cast<uint16_t *>(lds.key)[e] = (uint16_t)key;
+            }
         } else if (kWaves > 1) {
             lds.bound[tid] = best;
         }
         row_sync<THREADS>();
         if (wave == 0) {
-            const uint32_t least = order_of(-INFINITY) >> 16;
-            uint32_t lo = least, hi = (order_of(most) >> 16) + 1;  // count reach lo, fewer hi
-            if (each) {
-                uint32_t two[kShort / 2 / kWave + 1];
-#pragma unroll
-                for (int k = 0; k < kShort / 2 / kWave; ++k) two[k] = reinterpret_cast<uint32_t *>(lds.key)[k * kWave + lane];
+            // the highest key that `count` reach; of f32 its upper half, and its lower half only where the
+            // upper one lets half as many again through, as it does if the logits have an offset in common
+            constexpr int kHalf = kWide ? 16 : 0;
+            auto search = [&](uint32_t lo, uint32_t hi, auto reach) {  // count reach lo, fewer hi
                 while (hi - lo > 1) {
                     const uint32_t mid = lo + (hi - lo) / 2;
-                    int reach = 0;
+                    (reach(mid) >= count ? lo : hi) = mid;
+                }
+                return lo;
+            };
+            const uint32_t least = key_of(-INFINITY, T());
+            const uint32_t top = (key_of(most, T()) >> kHalf) + 1;
+            uint32_t key;
+            if (each) {
+                const uint32_t *keys = reinterpret_cast<const uint32_t *>(lds.key);
+                uint32_t word[kWords / kWave];
 #pragma unroll
-                    for (int k = 0; k < kShort / 2 / kWave; ++k)
-                        reach += __popcll(__ballot(two[k] >> 16 >= mid)) + __popcll(__ballot((two[k] & 0xffffu) >= mid));
-                    (reach >= count ? lo : hi) = mid;
+                for (int k = 0; k < kWords / kWave; ++k) word[k] = keys[k * kWave + lane] >> kHalf;
+                auto reach = [&](uint32_t limit) {
+                    int n = 0;
+#pragma unroll
+                    for (int k = 0; k < kWords / kWave; ++k) {
+                        n += __popcll(__ballot((kWide ? word[k] : word[k] >> 16) >= limit));
+                        if (!kWide) n += __popcll(__ballot((word[k] & 0xffffu) >= limit));
+                    }
+                    return n;
+                };
+                key = search(least >> kHalf, top, reach);
+                if (kWide && reach(key) > count + count / 2 + 8) {
+#pragma unroll
+                    for (int k = 0; k < kWords / kWave; ++k) word[k] = keys[k * kWave + lane];
+                    key = search(key << 16, (key + 1) << 16, reach);
+                } else {
+                    key <<= kHalf;
                 }
             } else {
                 uint32_t own[kWaves];
 #pragma unroll
-                for (int k = 0; k < kWaves; ++k) own[k] = order_of(kWaves > 1 ? lds.bound[k * kWave + lane] : best) >> 16;
-                while (hi - lo > 1) {
-                    const uint32_t mid = lo + (hi - lo) / 2;
-                    int reach = 0;
+                for (int k = 0; k < kWaves; ++k) own[k] = key_of(kWaves > 1 ? lds.bound[k * kWave + lane] : best, T()) >> kHalf;
+                auto reach = [&](uint32_t limit) {
+                    int n = 0;
 #pragma unroll
-                    for (int k = 0; k < kWaves; ++k) reach += __popcll(__ballot(own[k] >= mid));
-                    (reach >= count ? lo : hi) = mid;
+                    for (int k = 0; k < kWaves; ++k) n += __popcll(__ballot(own[k] >= limit));
+                    return n;
+                };
+                key = search(least >> kHalf, top, reach);
+                if (kWide && reach(key) > count + count / 2 + 8) {
+#pragma unroll
+                    for (int k = 0; k < kWaves; ++k) own[k] = key_of(kWaves > 1 ? lds.bound[k * kWave + lane] : best, T());
+                    key = search(key << 16, (key + 1) << 16, reach);
+                } else {
+                    key <<= kHalf;
                 }
             }
-            bound = lo == least ? -INFINITY : of_order(lo << 16);
+            bound = key <= least ? -INFINITY : of_key(key, T());
             if (kWaves > 1 && lane == 0) lds.bound[THREADS - 1] = bound;  // read by this wave already
         }
         row_sync<THREADS>();
         if (kWaves > 1) bound = lds.bound[THREADS - 1];
     }
     if (__ballot(best >= bound) != 0) {
-        const float least = cut(bound);
         uint32_t left = 0;  // the thread's vectors that may hold a logit that reaches the bound
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (i * THREADS * V - skew < len) left |= (tops.get(i) >= least ? 1u : 0u) << i;
+            if (i * THREADS * V - skew < len) left |= (tops.get(i, r.raw[i]) >= bound ? 1u : 0u) << i;
         while (__ballot(left != 0) != 0) {
             const int first = ((__ffs(left) - 1) * THREADS + tid) * V - skew;
             const int at = append(left != 0 && first < len, &lds.vectors);
@@ -710,7 +777,7 @@ __global__ void __launch_bounds__(kBlock<THREADS>, (kWavesPerSimd<THREADS, NV>))
     if (teach) u_max = load_teacher_logits<T, THREADS>(job, row, q);
 
     float best = -INFINITY;
-    VectorTops<NV> tops;
+    VectorTops<T, NV> tops;
     r.each_raw([&](int i, const u32x4 &x) {
         const float top = vector_max(x, T());
         if (TOP) tops.set(i, top);
@@ -756,7 +823,7 @@ __global__ void __launch_bounds__(kBlock<THREADS>, (kWavesPerSimd<THREADS, NV>))
             if (regular) {
                 float *value = job.part_value + part * job.a.count;
                 int *token = job.part_token + part * job.a.count;
-                find_top<T, THREADS, NV>(tops, z, len, r.skew, job.a.count, best, a.m, lds, [&](int rank, float v, int at) {
+                find_top<T, THREADS, NV>(r, tops, z, len, job.a.count, best, a.m, lds, [&](int rank, float v, int at) {
                     value[rank] = v;
                     token[rank] = begin + at;
                 });
@@ -772,7 +839,7 @@ __global__ void __launch_bounds__(kBlock<THREADS>, (kWavesPerSimd<THREADS, NV>))
             if (regular) {
                 const float log_sum = stats_log_sum(a), inv_temp = job.inv_temp, m = a.m;
                 const bool some = a.s != 0.0f;
-                find_top<T, THREADS, NV>(tops, z, len, r.skew, job.a.count, best, a.m, lds, [&](int rank, float v, int at) {
+                find_top<T, THREADS, NV>(r, tops, z, len, job.a.count, best, a.m, lds, [&](int rank, float v, int at) {
                     value[rank] = some ? (v - m) * inv_temp - log_sum : -INFINITY;
                     token[rank] = at;
                 });

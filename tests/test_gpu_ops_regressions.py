@@ -38,3 +38,47 @@ def test_results_can_be_changed_in_place(how):
     scores = ops.token_log_probs(z, tokens)
     (scores.log_probs * mask - 0.1 * scores.entropy).sum().backward()
     assert torch.equal(got, z.grad)
+
+
+def _us(call, calls=10, rounds=5):
+    """The smallest time of a call over a few rounds, back to back."""
+    call()
+    best = float("inf")
+    for _ in range(rounds):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(calls):
+            call()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3 / calls)
+    return best
+
+
+@pytest.mark.parametrize("rows,v", [(1, 32000), (1024, 32000), (8192, 4000), (256, 131072), (4096, 12000), (2048, 1000), (2048, 500)])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_alternatives_of_rows_with_an_offset(rows, v, dtype):
+    """An offset common to a row's logits changes neither the alternatives nor what the search for them
+    costs: its bound and the vectors' largest logits were cut to 16 bits of f32 once, which most of such
+    a row reached (up to 12 times as long; three times is allowed). The logits lie on steps that every
+    offset keeps."""
+    _need_gpu()
+    from luminamoon_amd import ops
+    from tests.ops_util import DTYPES
+
+    g = torch.Generator().manual_seed(v)
+    step = 2.0 ** -10 if dtype == "f32" else 0.5
+    base = ((torch.randn(min(rows, 64), v, generator=g) / step).round() * step).cuda()
+    base = base[torch.arange(rows, device="cuda") % base.shape[0]]
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    for top in (8, 20, 64, 128):
+        here = {}
+        for offset in (0.0, 500.0, -1000.0):
+            z = (base + offset).to(DTYPES[dtype])
+            print(f"[case] {rows}x{v} {dtype} top {top} offset {offset}", flush=True)
+            out = ops.token_log_probs_forward(z, tokens, top=top)
+            want = torch.sort(z[:64].double(), dim=-1, descending=True, stable=True).indices[:, :top]
+            assert torch.equal(out.top_tokens[:64], want)
+            here[offset] = _us(lambda: ops.token_log_probs_forward(z, tokens, top=top))
+        print(f"[time] {rows}x{v} {dtype} top {top} {here}", flush=True)
+        assert max(here.values()) < 3 * here[0.0], here
