@@ -82,3 +82,40 @@ def test_alternatives_of_rows_with_an_offset(rows, v, dtype):
             here[offset] = _us(lambda: ops.token_log_probs_forward(z, tokens, top=top))
         print(f"[time] {rows}x{v} {dtype} top {top} {here}", flush=True)
         assert max(here.values()) < 3 * here[0.0], here
+
+
+def _graph_us(call, calls=20, replays=5):
+    """A call's time on the GPU alone: the smallest of a few replays of many in a graph."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(calls):
+            call()
+    return min(_us(graph.replay, calls=1) for _ in range(replays)) / calls
+
+
+@pytest.mark.parametrize("rows,d,one_row", [(32, 768, 8), (4, 16384, 1), (4, 8192, 1), (64, 256, 16)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_layer_norm_gradient_of_x_alone_uses_more_than_one_block(rows, d, one_row, dtype):
+    """With frozen weights no columns' sums are wanted, and rows spread over blocks; one block walked
+    them all before. A block has as many rows as it takes at a time: all take as long as one such block,
+    where a walk takes two to three times that (1.6 is allowed). The gradient is the same to the bit."""
+    _need_gpu()
+    from luminamoon_amd import ops
+    from tests.ops_util import DTYPES
+
+    g = torch.Generator().manual_seed(d)
+    x, dy = (torch.randn(rows, d, generator=g).to(DTYPES[dtype]).cuda() for _ in range(2))
+    w = torch.randn(d, generator=g).cuda()
+    _, mean, rstd = ops.layer_norm_forward(x, w)
+    dx = ops.layer_norm_backward(dy, x, w, mean, rstd, True, False, False)[0]
+    assert torch.equal(dx, ops.layer_norm_backward(dy, x, w, mean, rstd)[0])
+    many = _graph_us(lambda: ops.layer_norm_backward(dy, x, w, mean, rstd, True, False, False))
+    few = [t[:one_row] for t in (dy, x, mean, rstd)]
+    one = _graph_us(lambda: ops.layer_norm_backward(few[0], few[1], w, few[2], few[3], True, False, False))
+    print(f"[time] {rows}x{d} {dtype} {many:.2f} us, {one_row} rows {one:.2f} us", flush=True)
+    assert many < 1.6 * one
