@@ -1218,10 +1218,15 @@ typedef void (*RowsKernel)(Job);
     ((dtype) == LV_DTYPE_F32 ? (RowsKernel)KERNEL<F32, ##__VA_ARGS__> \
      : (dtype) == LV_DTYPE_BF16 ? (RowsKernel)KERNEL<BF16, ##__VA_ARGS__> : (RowsKernel)KERNEL<F16, ##__VA_ARGS__>)
 
+// The kernel of a cut, of those that cuts of such a call can have: 256 threads with sixteen vectors come
+// without a gradient only, 1024 with sixteen with one (or on the way to one).
 template <typename T, Way WAY, bool TOP, bool GRAD>
 static RowsKernel pick_rows(const Cut &c) {
     if constexpr (!GRAD) {
         if (c.threads == 256 && c.vectors == 16) return rows_kernel<T, 256, 16, WAY, TOP, GRAD>;
+    }
+    if constexpr (WAY == kDistill) {
+        if (c.threads == 1024 && c.vectors == 16) return rows_kernel<T, 1024, 16, WAY, TOP, GRAD>;
     }
     switch (c.threads * 100 + c.vectors) {
     case 6404: return rows_kernel<T, 64, 4, WAY, TOP, GRAD>;
@@ -1230,7 +1235,7 @@ static RowsKernel pick_rows(const Cut &c) {
     case 51208: return rows_kernel<T, 512, 8, WAY, TOP, GRAD>;
     case 51213: return rows_kernel<T, 512, 13, WAY, TOP, GRAD>;
     case 102408: return rows_kernel<T, 1024, 8, WAY, TOP, GRAD>;
-    default: return rows_kernel<T, 1024, 16, WAY, TOP, GRAD>;
+    default: return nullptr;
     }
 }
 
@@ -1242,6 +1247,7 @@ static RowsKernel pick_rows(int dtype, const Cut &c) {
 }
 
 static int run(RowsKernel k, int64_t blocks, int threads, size_t lds, const Job &job, hipStream_t s, const char *what) {
+    if (k == nullptr) return fail(LV_STATUS_EXECUTION_FAILED, "%s: no kernel of %d threads a row for this cut", what, threads);
     k<<<dim3((unsigned)blocks), dim3((unsigned)threads), lds, s>>>(job);
     return launched(what);
 }
