@@ -6,8 +6,13 @@
  * Plain pointers and sizes only. Every pointer is a device (HBM) pointer on the current HIP device;
  * `stream` is a hipStream_t passed as void* (NULL = default stream). Calls are asynchronous on
  * `stream`, allocate nothing and wait for nothing, so they can be captured into a HIP graph.
- * Sums and statistics are f32 whatever the tensors' type; every result is a fixed function of the
- * inputs (no atomics whose order could change it).
+ * Sums and statistics are f32 whatever the tensors' type. A call repeated on the same memory gives the
+ * same bits: no result depends on the order of atomics or on timing. Layer norm's rows give the same
+ * bits anywhere and in any number; its columns' sums depend on the number of rows. Over rows of logits
+ * the most likely tokens and the largest logit are the same everywhere, but the last bits of what is
+ * summed over a row depend on the number of rows, which decides how a row is cut, and for 16-bit logits
+ * on the half of a 4-byte word that the row begins at: equal rows of an odd vocabulary may differ in
+ * them between even and odd row numbers, and a packed copy from a view.
  *
  * Matrices are rows x width, elements of a row contiguous, rows `*_stride` elements apart, at any
  * element offset (no alignment beyond the element's own).
