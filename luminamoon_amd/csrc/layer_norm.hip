@@ -10,13 +10,15 @@
 // partial row of each, and a second kernel adds those in a fixed order. Where a group has four rows at
 // most, one block takes them all and writes the sums itself.
 //
-// What bounds it: memory, once there are rows enough. 32768 x 4096 bf16 takes 83 us forward (6.4 TB/s)
-// and 146 us backward (5.5 TB/s, 7.7 us of it the second kernel; 17 MB of partial rows), a large copy
-// runs at 6.15. 174762 x 768 bf16: 87 us (6.2) and 154 (5.2). Blocks therefore walk many rows, so that
-// weights are read once a block and the next row is under way while one is worked on. Small calls are
-// bound by the launches: 8192 x 768 f32 takes 9.7 us, 16384 x 768 bf16 backward 21.4 with 3.9 of them the
-// second kernel, one row 3.4 and the host's part of the call 6.4. Rows of odd 16-bit widths start half
-// way into a word and take a fifth to a quarter longer (131200 x 1023: 107 us, 131072 x 1024: 85).
+// What bounds it: memory, once there are rows enough. 32768 x 4096 bf16 takes 84 us forward, back to back,
+// where the last of its output is still in the 256 MiB cache as a call ends (95 us, 5.7 TB/s, with stores
+// past that cache), and 145 us backward (5.5 TB/s, 7.5 us of it the second kernel; 17 MB of partial
+// rows); a large copy runs at 6.15. 174762 x 768 bf16: 88 us (94 past the cache) and 154 (5.2). Blocks
+// therefore walk many rows, so that weights are read once a block and the next row is under way while one
+// is worked on. Small calls are bound by the launches: 8192 x 768 f32 takes 9.7 us, 16384 x 768 bf16
+// backward 21.4 with 3.9 of them the second kernel, one row 3.4 and the host's part of the call 6.4. Rows
+// of odd 16-bit widths start half way into a word and take a fifth to a quarter longer (131200 x 1023:
+// 110 us, 131072 x 1024: 85).
 // Rows above 16384 elements: 3.1 TB/s forward, 1.9 backward (6710 x 20000 bf16).
 #include "ops_common.h"
 
@@ -206,7 +208,9 @@ __global__ void __launch_bounds__(256) ln_forward_wide(LnJob job) {
 
 // Groups of TPR threads (8 to 1024) walk the rows, each thread its NV vectors of every row; the next row's vectors
 // are under way while one is worked on. Per row the group's two sums cost one barrier (none for a
-// wave), and x and dy are unpacked twice rather than kept unpacked across it.
+// wave), and x and dy are unpacked twice rather than kept unpacked across it. Four waves a SIMD leave 128
+// registers: f32 rows above 512 columns and 16-bit rows above 4096 spill 4 to 20 of them (32768 x 4096 f32
+// 286 us, 5.6 TB/s; 16384 x 768 f32 31.8, 4.7; 16384 x 8192 bf16 161, 5.0).
 template <typename T, typename W, int TPR, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS, 4) ln_backward(LnJob job) {
     constexpr int V = Type<T>::kVec, kGroups = THREADS / TPR, kWaves = TPR / kWave, kLanes = TPR < kWave ? TPR : kWave;

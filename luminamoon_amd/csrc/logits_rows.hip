@@ -18,13 +18,15 @@
 // holds (many equal logits, fewer finite ones than alternatives, or large ones crowded into few
 // threads), the exact count-th one is found first, by bisection of its value and then of its index.
 //
-// What bounds it: reading the logits (6.4 TB/s for 8192 rows of 32000 bf16 without alternatives) and,
+// What bounds it: reading the logits (6.5 TB/s for 8192 rows of 32000 bf16 without alternatives) and,
 // with the gradient, writing as much (5.6 TB/s); a large copy runs at 6.15. With alternatives
-// instruction issue joins it: 8192 x 50257 bf16 with 8 takes 12.7 vector instructions a logit, 80% of the
-// SIMDs' cycles, 152 us (5.4 TB/s). Eight vectors a thread fit 64 registers, so a compute unit holds 256
-// KiB of rows at once, several rows in different phases: 512 threads a row keep the memory busier than
-// 1024 (8192 x 32000: 82 and 116 us). Short rows and few rows are bound by the way through the steps:
-// 7.0 us for one row of 32000, 8.3 with 20 alternatives, 16.3 for 257 rows f32 with 64.
+// instruction issue joins it: 8192 x 50257 bf16 with 8 takes 12.7 vector instructions a logit, 80 to 89% of
+// the SIMDs' cycles, 149 us (5.5 TB/s) at a stride of 50304 and 155 packed. Eight vectors a thread fit 64
+// registers, so a compute unit holds 256 KiB of rows at once, several rows in different phases: 512 threads
+// a row keep the memory busier than 1024 (8192 x 32000: 81 and 112 us). Short rows and few rows are bound
+// by the way through the steps: one row of 32000 bf16 with 20 alternatives keeps its block for 7.4 us,
+// 257 rows of 32000 f32 with 64 take 16.3. Rows with fewer finite logits than alternatives are read
+// thirty times: 8192 x 32000 bf16 with 20 takes 93 us, and 2316 where 5 logits are finite.
 #include "ops_common.h"
 
 #include <cfloat>
@@ -127,7 +129,7 @@ struct RowLds {
 };
 // Alternatives that a single wave's row is searched for: its bound is the less tight the more they are
 // of its 64 threads (some 88 logits reach the bound for 48, 177 for 60, more than its list holds).
-// 65536 rows of 1000 bf16 with 48: 134 us by single waves, 240 by blocks of 256.
+// 65536 rows of 1000 bf16 with 48: 124 us by single waves, 204 by blocks of 256.
 constexpr int kMostOfAWave = 48;
 
 // The sum over the row's threads of each of N values, the same in every thread. Consecutive calls
@@ -194,8 +196,8 @@ static __device__ __forceinline__ float vector_max(const u32x4 &r, F16) {
 
 // A row (or slice) z[0, len) over THREADS threads, NV vectors each: thread t holds vectors t,
 // t + THREADS, ... A 16-bit row that starts half way into a 4-byte word has its vectors one logit
-// earlier (`skew`), on words: 8192 rows of 50257 bf16, every second of them off, take 150 us this way
-// and 176 with loads off their words. Logits before the row and past its end are -inf.
+// earlier (`skew`), on words: 8192 rows of 50257 bf16, every second of them off, take 155 us this way
+// and 179 with loads off their words (with 8 alternatives). Logits before the row and past its end are -inf.
 template <typename T, int THREADS, int NV>
 struct RowRegisters {
     static constexpr int V = Type<T>::kVec;
@@ -433,8 +435,8 @@ static __device__ __forceinline__ void find_top(RowRegisters<T, THREADS, NV> &r,
         bound = -wave_max(-pick);
     } else {
         // A short row gives too few threads' bests for a bound: there every logit stands for itself, for
-        // twice the time (65536 rows of 1000 bf16 with 64 alternatives take 244 us, 432 this way; with
-        // 128 they take 495 us this way, 1143 with the exact search that a bound of -inf leads to).
+        // twice the time (65536 rows of 1000 bf16 with 64 alternatives take 240 us, 424 this way; with
+        // 128 they take 484 us this way, 1106 with the exact search that a loose bound leads to).
         constexpr bool kWide = sizeof(store_t<T>) == 4;  // a key fills a word, or half of one
         constexpr int kWords = Lds::kLogits * 2;         // of the keys where the list will be
         constexpr int kShort = kWaves == 4 && NV <= 8 ? kWords * (kWide ? 1 : 2) : 0;
@@ -680,7 +682,9 @@ static __device__ __forceinline__ float grad_weight(const Job &job, int64_t row)
 }
 
 // The teacher's tokens in [begin, end) of a row's gradient, by the row's threads: w (p - q) over the
-// w p that they wrote there before their last meeting. sum: of the entries' e.
+// w p that they wrote there before their last meeting. sum: of the entries' e. Every entry is compared
+// with all of them for doubled tokens, quadratic in their number: the step of 4096 x 32000 bf16 takes 94
+// us with 1, 99 with 32, 115 with 128, 219 with 512 and 630 with 1024.
 template <typename T, int THREADS>
 static __device__ __forceinline__ void grad_of_teacher(const Job &job, int64_t row, const RowStats &a, const Teacher &q, float sum,
                                                        float w, int begin, int end) {
@@ -1087,10 +1091,10 @@ static int round_up(int64_t n, int m) { return (int)((n + m - 1) / m * m); }
 
 // What holds a row: threads and 16-byte vectors of each, smallest first. In us, without and with 8
 // alternatives and the distillation step, bf16:
-//   32768 x 4000   64 x 8: 45, 62, 127     256 x 4: 66, 109, 140
-//   16384 x 12000  256 x 8: 62, 86, 158    512 x 4: 85, 130, 170
-//   8192 x 32000   512 x 8: 82, 111, 190   256 x 16: 83, 97, 197    1024 x 4: 116, 157, 234
-//   8192 x 50257   512 x 13: 137, 161, 327 1024 x 8: 169, 214, 335  256 x 25: 135, 198, 340
+//   32768 x 4000   64 x 8: 42, 55, 115     256 x 4: 61, 106, 138
+//   16384 x 12000  256 x 8: 62, 82, 156    512 x 4: 80, 128, 168
+//   8192 x 32000   512 x 8: 81, 100, 188   256 x 16: 80, 90, 197    1024 x 4: 112, 151, 231
+//   8192 x 50257   512 x 13: 136, 155, 327 1024 x 8: 160, 206, 344  256 x 25: 130, 152, 340
 static const int kShapes[][2] = {{64, 4}, {64, 8}, {256, 8}, {512, 8}, {512, 13}, {1024, 8}, {1024, 16}};
 constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0];
 constexpr int kSliced = 3;  // the shape of slices: 512 threads, 8 vectors
@@ -1104,8 +1108,9 @@ static int row_skew(const lv_logits_args *a) {
 // The smallest block that holds a whole row. Longer rows are cut into slices of the largest block's,
 // or of the smallest one's that still give every compute unit a block. Without a gradient, which
 // would have to read the row again, rows are cut to slices of 512 threads where they would take 1024
-// threads and 16 vectors (2048 x 50257 f32: 92 us whole, 75 cut), or 8 and there are many rows
-// (4096 x 65536 bf16 with 8 alternatives: 129 and 116 us, as slices of 512 threads; 512 rows: 22 and 25).
+// threads and 16 vectors (2048 x 50257 f32: 86 us whole, 62 cut), or 8 and there are many rows
+// (4096 x 65536 bf16 with 8 alternatives: 116 us whole and 105 as slices of 512 threads, which cut_rows
+// makes 256, 98 us; 512 rows: 20 whole and 22).
 static Cut smallest_block(const lv_logits_args *a, int top, int skew, bool grad) {
     const int64_t vocab = (int64_t)a->vocab, rows = (int64_t)a->rows;
     const int v = a->dtype == LV_DTYPE_F32 ? 4 : 8;
@@ -1133,10 +1138,10 @@ static Cut smallest_block(const lv_logits_args *a, int top, int skew, bool grad)
 // Half the threads with twice the vectors hold as much as 512 with 8. Without a gradient and with eight
 // blocks or more for every compute unit they are quicker, as the threads meet and search in half the
 // waves, but for slices without alternatives. In us, 512 x 8 and 256 x 16, with 8 alternatives (without):
-//   8192 x 32000 bf16 106, 91 (79, 80)   8192 x 18000 bf16 80, 67 (57, 48)   2048 x 32000 bf16 34, 33 (29, 29)
-//   1024 x 32000 bf16 19.9, 20.6 (16.3, 17.4)   8192 x 12000 f32 74, 65 (61, 61)
-//   slices: 4096 x 60000 f16 110, 93 (84, 84)   2048 x 131072 bf16 112, 102 (87, 92)
-// The distillation step of 8192 x 32000 takes 188 and 196.
+//   8192 x 32000 bf16 100, 90 (81, 80)   8192 x 18000 bf16 77, 62 (54, 46)   2048 x 32000 bf16 30, 28 (23, 24)
+//   1024 x 32000 bf16 17.6, 18.4 (14.2, 15.0)   8192 x 12000 f32 70, 61 (60, 60)
+//   slices: 4096 x 60000 f16 100, 88 (80, 81)   2048 x 131072 bf16 102, 94 (85, 89)
+// The distillation step of 8192 x 32000 takes 188 and 197.
 static Cut cut_rows(const lv_logits_args *a, int top, int skew, bool grad) {
     Cut c = smallest_block(a, top, skew, grad);
     if (!grad && c.threads == 512 && c.vectors == 8 && (top > 0 || c.slices == 1) && (int64_t)a->rows * c.slices >= 8 * compute_units())

@@ -1,4 +1,4 @@
-"""The operators in autograd."""
+"""The operators in autograd: reverse mode of the first order. Double backward, forward mode and vmap raise."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
@@ -32,7 +32,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 
 class LayerNorm(torch.nn.Module):
-    """`layer_norm` with its parameters; a stand-in for torch.nn.LayerNorm over one axis."""
+    """`layer_norm` with its parameters, named as torch.nn.LayerNorm's over one axis. There is a weight always,
+    and the result has x's dtype, also under autocast (where torch's is float32)."""
 
     def __init__(self, width: int, eps: float = 1e-5, bias: bool = True, device=None, dtype=None) -> None:
         super().__init__()
